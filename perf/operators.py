@@ -12,7 +12,6 @@ Quantized tensors are handed back as the values they stand for, in bfloat16, whi
 
 from __future__ import annotations
 
-import functools
 import math
 
 import torch
@@ -216,50 +215,49 @@ def _plain(state):
 # ---- the package's operators
 
 
-@functools.lru_cache(maxsize=None)
-def _package():
-    """The functions as a program has them that imported them where it begins."""
-    from types import SimpleNamespace
-
-    from kohakuwullm_amd.kernels import elementwise, mxfp4, mxfp8
-    from kohakuwullm_amd.kernels.mxfp8 import fused_act
-
-    return SimpleNamespace(add_rms_norm=elementwise.add_rms_norm, add_rmsnorm_mx=fused_act.add_rmsnorm_mx, quantize_mx=mxfp8.quantize_mx,
-                           **{name: getattr(mxfp4, name) for name in mxfp4.__all__})
-
-
 def _own(state):
-    p = _package()
+    from kohakuwullm_amd.kernels.elementwise import add_rms_norm
+    from kohakuwullm_amd.kernels.mxfp4 import (
+        dequantize_mx,
+        grouped_mxfp4_gemm,
+        mxfp4_linear,
+        mxfp4_matmul_pq,
+        quantize_mxfp4,
+        quantize_mxfp4_cols,
+    )
+    from kohakuwullm_amd.kernels.mxfp8 import quantize_mx
+    from kohakuwullm_amd.kernels.mxfp8.fused_act import add_rmsnorm_mx
+
     case = state["case"]
     if case["kind"] == "norm":
         x, r, w = state["x"], state["r"], state["w"]
         if case["mode"] == "codes":
-            h, q, s = p.add_rmsnorm_mx(x, r, w, EPS)
-            return [h, p.dequantize_mx(q, s, torch.bfloat16)]
+            h, q, s = add_rmsnorm_mx(x, r, w, EPS)
+            return [h, dequantize_mx(q, s, torch.bfloat16)]
         if case["mode"] == "plain":
             with torch.no_grad():
-                return list(p.add_rms_norm(x, r, w, EPS))
+                return list(add_rms_norm(x, r, w, EPS))
         leaves = [t.detach().requires_grad_() for t in (x, r, w)]
-        outputs = p.add_rms_norm(*leaves, EPS)
+        outputs = add_rms_norm(*leaves, EPS)
         torch.autograd.backward(outputs, [state["dout"], state["dh"]])
         return [t.detach() for t in outputs] + [t.grad for t in leaves]
     if case["kind"] == "quantize":
         x = state["x"]
-        out = [p.dequantize_mx(*p.quantize_mxfp4(x), torch.bfloat16)]
-        return out + [p.dequantize_mx(*p.quantize_mxfp4_cols(x), torch.bfloat16)] if case["axes"] == "both" else out
+        out = [dequantize_mx(*quantize_mxfp4(x), torch.bfloat16)]
+        return out + [dequantize_mx(*quantize_mxfp4_cols(x), torch.bfloat16)] if case["axes"] == "both" else out
     if case["kind"] == "linear":
         if not case["train"]:
             with torch.no_grad():
-                return [p.mxfp4_linear(state["x"], state["operands"])]
+                return [mxfp4_linear(state["x"], state["operands"])]
         x, w = state["x"].detach().requires_grad_(), state["w"].detach().requires_grad_()
-        y = p.mxfp4_linear(x, state["operands"], w)
+        y = mxfp4_linear(x, state["operands"], w)
         y.backward(state["dout"])
         return [y.detach(), x.grad, w.grad]
     if case["kind"] == "product":
-        q, s = p.quantize_mxfp4(state["x"])
-        return [p.mxfp4_matmul_pq(q, s, state["wq"], state["ws"], _DTYPES[case["result"]])]
-    q, s = p.quantize_mx(state["x"])
-    return [p.grouped_mxfp4_gemm(q, s, state["wq"], state["ws"], state["offsets"], state["token_of"], out_dtype=state["x"].dtype)]
+        q, s = quantize_mxfp4(state["x"])
+        return [mxfp4_matmul_pq(q, s, state["wq"], state["ws"], _DTYPES[case["result"]])]
+    q, s = quantize_mx(state["x"])
+    return [grouped_mxfp4_gemm(q, s, state["wq"], state["ws"], state["offsets"], state["token_of"], out_dtype=state["x"].dtype)]
 
 
 def run(state):
