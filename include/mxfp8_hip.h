@@ -725,7 +725,8 @@ int mx_turn_bytes(const uint8_t *x, int64_t rows, int64_t cols, int64_t ldx, uin
 
 /*
  * C (M,N) = deq(A) deq(B)^T with B (N,K) in e2m1 and A (M,K) in a_format, fp32 sums.  lda and ldb are bytes; code rows start on
- * 16-byte boundaries (MX_EUNSUPPORTED otherwise).  K % 32 == 0.  workspace as in mx_gemm_nt: without one no tile is cut along K.
+ * 16-byte boundaries (MX_EUNSUPPORTED otherwise).  K % 32 == 0; M, N and K up to 2^31 - 1024 (MX_EUNSUPPORTED above), here and
+ * in the two entries below.  workspace as in mx_gemm_nt: without one no tile is cut along K.
  */
 int mx_fp4_gemm_nt(const uint8_t *aq, const uint8_t *a_scale, int a_format, const uint8_t *bq, const uint8_t *b_scale, void *c,
                    int c_dtype, int64_t M, int64_t N, int64_t K, int64_t lda, int64_t ldas, int64_t ldb, int64_t ldbs, int64_t ldc,

@@ -85,7 +85,7 @@ extern "C" int mx_fp4_activation_gemm_nt(const void *x, int x_dtype, int64_t ldx
     if ((c_dtype != MX_BF16 && c_dtype != MX_FP16) || (x_dtype != c_dtype && x_dtype != MX_FP32)) return MX_EUNSUPPORTED;
     if (M == 0 || N == 0) return MX_OK;
     if (!c || (K && (!x || !bq || !b_scale))) return MX_EINVAL;
-    if (K == 0 || !activation_rows_ok(M, K) || !few_aligned(x, 16) || ldx * (x_dtype == MX_FP32 ? 4 : 2) % 16 || !few_aligned(bq, 16) || ldb % 16)
+    if (K == 0 || N > FP4_EXTENT || !activation_rows_ok(M, K) || !few_aligned(x, 16) || ldx * (x_dtype == MX_FP32 ? 4 : 2) % 16 || !few_aligned(bq, 16) || ldb % 16)
         return MX_EUNSUPPORTED;
     hipStream_t st = (hipStream_t)stream;
     if (stream_is_capturing(st)) return MX_ECAPTURE;

@@ -21,6 +21,9 @@ struct Fp4GemmArgs {
     float *slice_ws;
 };
 
+// The longest M, N and K: the kernels add a stage, a tile or a loop's stride (1024 at most) to a row, column or place in K in 32 bits.
+constexpr int64_t FP4_EXTENT = ((int64_t)1 << 31) - 1024;
+
 // Where expert e's rows begin (e = E: end): inside the matrix whatever the table says.
 __device__ __forceinline__ int group_bound(const Fp4GemmArgs &a, int e) {
     const int at = a.offsets[e];

@@ -176,7 +176,7 @@ extern "C" int mx_fp4_gemm_nt(const uint8_t *aq, const uint8_t *a_scale, int a_f
         return MX_EINVAL;
     if (M == 0 || N == 0) return MX_OK;
     if (!c || (K && (!aq || !a_scale || !bq || !b_scale))) return MX_EINVAL;
-    if (K && (!codes_ok(aq, lda) || !codes_ok(bq, ldb))) return MX_EUNSUPPORTED;
+    if (M > FP4_EXTENT || N > FP4_EXTENT || K > FP4_EXTENT || (K && (!codes_ok(aq, lda) || !codes_ok(bq, ldb)))) return MX_EUNSUPPORTED;
     hipStream_t st = (hipStream_t)stream;
     if (mx::stream_is_capturing(st)) return MX_ECAPTURE;
     const Fp4GemmArgs a = {aq, a_scale, bq, b_scale, nullptr, nullptr, c, lda, ldas, 0, ldb, 0, ldbs, ldc, (int)M, (int)N, (int)K, 1, (int)M};
@@ -194,7 +194,8 @@ extern "C" int mx_fp4_grouped_gemm_nt(const uint8_t *xq, const uint8_t *x_scale,
     if (M == 0 || N == 0) return MX_OK;
     if (!offsets || !out || (K && (!xq || !x_scale || !wq || !w_scale))) return MX_EINVAL;
     if ((!index && x_rows < M) || x_rows == 0) return MX_EINVAL;
-    if (K && (!codes_ok(xq, ldx) || !codes_ok(wq, ldw) || stride_we % 16)) return MX_EUNSUPPORTED;
+    if (M > FP4_EXTENT || N > FP4_EXTENT || K > FP4_EXTENT || (K && (!codes_ok(xq, ldx) || !codes_ok(wq, ldw) || stride_we % 16)))
+        return MX_EUNSUPPORTED;
     hipStream_t st = (hipStream_t)stream;
     if (mx::stream_is_capturing(st)) return MX_ECAPTURE;
     const Fp4GemmArgs a = {xq, x_scale, wq, w_scale, index, offsets, out, ldx, ldxs, stride_we, ldw, stride_wse, ldws, ldo, (int)M, (int)N, (int)K, (int)E, (int)x_rows};
