@@ -743,7 +743,8 @@ int mx_fp4_activation_gemm_nt(const void *x, int x_dtype, int64_t ldx, const uin
 /*
  * out[m] = deq(x[index[m] or m]) deq(w[e(m)])^T for rows sorted by expert, offsets (E+1) as in mx_grouped_gemm_nt; w (E,N,K) in
  * e2m1, x (x_rows,K) in x_format.  ldx, ldw, stride_we are bytes.  Rows of out outside every expert's range are not written, or
- * set to zero (zero_rest).  Offsets and indices that lie outside M and x_rows are taken to the nearest row inside.
+ * set to zero (zero_rest).  Offsets and indices that lie outside M and x_rows are taken to the nearest row inside; of offsets that
+ * decrease it is left open which rows are written, nothing outside the operands is touched.
  */
 int mx_fp4_grouped_gemm_nt(const uint8_t *xq, const uint8_t *x_scale, int x_format, int64_t x_rows, int64_t ldx, int64_t ldxs,
                            const int32_t *index, const uint8_t *wq, const uint8_t *w_scale, int64_t stride_we, int64_t ldw,

@@ -48,7 +48,8 @@ __device__ __forceinline__ void store_value(void *c, int64_t at, float v) {
 __host__ __device__ __forceinline__ int fp4_slice_stages(int KT, int slices) { return ((KT + slices - 1) / slices + 3) & ~3; }
 
 // Row tiles of the experts before e, for e in [0, E]: a workgroup's first wave builds them once, so that the expert of a row tile is a
-// search in LDS instead of a walk over the offsets in memory.
+// search in LDS instead of a walk over the offsets in memory.  Offsets that never decrease make tiles_m of them at most, and what numbers
+// tiles counts on that (plan_fp4_tiles, stream_takes): the table ends there whatever the offsets say.
 constexpr int FP4_EXPERTS = 1024;  // more go to the kernel without tables
 __device__ __forceinline__ void build_tile_table(int *table, const Fp4GemmArgs &a, int rows) {
     if (threadIdx.x < 64) {
@@ -59,8 +60,8 @@ __device__ __forceinline__ void build_tile_table(int *table, const Fp4GemmArgs &
             const int n = e < a.E ? group_bound(a, e + 1) - group_bound(a, e) : 0;
             const int tiles = n > 0 ? (n + rows - 1) / rows : 0;
             const int upto = wave_incl_scan(tiles, lane);
-            if (e < a.E) table[e] = before + upto - tiles;
-            before += __shfl(upto, 63, 64);
+            if (e < a.E) table[e] = min(before + upto - tiles, a.tiles_m);
+            before = min(before + __shfl(upto, 63, 64), a.tiles_m);
         }
         if (lane == 0) table[a.E] = before;
     }
