@@ -13,6 +13,7 @@ import ctypes
 import os
 
 import torch
+from torch.autograd import forward_ad
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libmxfp8_hip.so")
@@ -285,6 +286,17 @@ def invoke(name: str, work: float, tensor: torch.Tensor, *args) -> None:
     end.record()
     check(status, name)
     TIMER.append((name, work, start, end))
+
+
+def recorded(*tensors: torch.Tensor | None) -> bool:
+    """Whether autograd records a gradient of a call on these tensors."""
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+def forward_mode() -> bool:
+    """Whether tensors may carry tangents.  A call that no gradient is recorded of still goes through its autograd function then, which
+    raises for a tangent that it would drop."""
+    return forward_ad._current_level >= 0
 
 
 def elsewhere(tensor: torch.Tensor) -> bool:

@@ -261,9 +261,10 @@ class _AddRMSNorm(torch.autograd.Function):
 
 
 def _add_norm(x, residual, weight, eps, quant):
-    if torch.is_grad_enabled() and (x.requires_grad or residual.requires_grad or (weight is not None and weight.requires_grad)):
-        if x.dim() and x.shape[-1] > ADD_NORM_BACKWARD_MAX:
-            raise ValueError(f"gradients need a row width of {ADD_NORM_BACKWARD_MAX} at most, got {x.shape[-1]}")
+    recorded = _lib.recorded(x, residual, weight)
+    if recorded and x.dim() and x.shape[-1] > ADD_NORM_BACKWARD_MAX:
+        raise ValueError(f"gradients need a row width of {ADD_NORM_BACKWARD_MAX} at most, got {x.shape[-1]}")
+    if recorded or _lib.forward_mode():
         return _AddRMSNorm.apply(x, residual, weight, eps, quant)
     out, h, _, q, s = launch_add_rmsnorm(x, residual, weight, eps, True, False, quant)
     return (out, h, q, s) if quant else (out, h)

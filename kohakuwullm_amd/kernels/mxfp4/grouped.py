@@ -139,11 +139,12 @@ def grouped_mxfp4_linear(x: torch.Tensor, operands, offsets: torch.Tensor, weigh
     shape = (wq.shape[0], wq.shape[1], x.shape[1])
     if weight is not None and weight.shape != shape:
         raise ValueError(f"weight {tuple(weight.shape)} does not match the quantized one {shape}")
-    if not torch.is_grad_enabled() or not (x.requires_grad or (weight is not None and weight.requires_grad)):
+    recorded = _lib.recorded(x, weight)
+    if not recorded and not _lib.forward_mode():
         return grouped_mxfp4_gemm(*quantize_mx(x), wq, ws, offsets, out_dtype=x.dtype, zero_rest=True)
-    if shape[1] % BLOCK_SCALE:
+    if recorded and shape[1] % BLOCK_SCALE:
         raise ValueError(f"gradients need a multiple of {BLOCK_SCALE} output columns, got {shape[1]}")
     wqt, wst = operands[2:] if len(operands) == 4 else (None, None)
-    if x.requires_grad and wqt is None:
+    if recorded and x.requires_grad and wqt is None:
         raise ValueError("the gradient of x needs the weights quantized along their output axis too: pass mxfp4_operands(weight)")
     return _GroupedMXFP4Linear.apply(x, weight, wq, ws, wqt, wst, offsets)

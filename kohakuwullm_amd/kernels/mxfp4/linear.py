@@ -96,8 +96,9 @@ def mxfp4_linear(x: torch.Tensor, operands, weight: torch.Tensor | None = None) 
     if len(operands) not in (2, 4):
         raise ValueError(f"operands are (q, s) or (q, s, qT, sT), got {len(operands)} tensors")
     wq, ws = operands[:2]
-    recorded = torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad))
-    if not recorded and (weight is None or weight.shape == (wq.shape[0], x.shape[-1])):
+    recorded = _lib.recorded(x, weight)
+    through = recorded or _lib.forward_mode()
+    if not through and (weight is None or weight.shape == (wq.shape[0], x.shape[-1])):
         made = host.fp4_linear(x, compute_dtype(x), wq, ws, False)
         if made is not None:
             return made[0]
@@ -109,12 +110,12 @@ def mxfp4_linear(x: torch.Tensor, operands, weight: torch.Tensor | None = None) 
     n, k = wq.shape[0], x.shape[-1]
     if weight is not None and weight.shape != (n, k):
         raise ValueError(f"weight {tuple(weight.shape)} does not match the quantized one ({n}, {k})")
-    if not recorded:
+    if not through:
         compute = compute_dtype(x)
         xq, xs, _, _ = quantized_activation(activation_matrix(x, compute), compute, False)
         return mxfp4_matmul_pq(xq, xs, wq, ws, compute).reshape(*x.shape[:-1], n)
     wqt, wst = operands[2:] if len(operands) == 4 else (None, None)
-    if x.requires_grad and wqt is None:
+    if recorded and x.requires_grad and wqt is None:
         raise ValueError("the gradient of x needs the weight quantized along its output axis too: pass mxfp4_operands(weight)")
     if wqt is not None and wqt.shape != (k, (n + -n % BLOCK_SCALE) // PAIR):
         raise ValueError(f"qT {tuple(wqt.shape)} is not the transposed copy of a weight ({n}, {k})")
