@@ -20,12 +20,14 @@ static int launch_few(Fp4GemmArgs a, hipStream_t st) {
 }
 
 // Parts of K by the workgroups of 16 columns there would be: see mx_fp4_few.h.  Rows of experts: two for short contractions, else four.
+// Activations are the same product with the same parts, of fewer columns (activations_pay).
 template <int CDT, int MT, int SRC>
 static int launch_few_parts(const Fp4GemmArgs &a, hipStream_t st) {
     const int64_t blocks = (a.N + 15) / 16, cus = num_cus();
     if (blocks <= 2 * cus) return launch_few<CDT, MT, 8, SRC>(a, st);
-    if constexpr (MT <= 2) {  // a wave stores one sub-tile
-        if (blocks > 8 * cus) return launch_few<CDT, MT, 2, SRC>(a, st);
+    if constexpr (MT <= (few_codes(SRC) ? 2 : 1)) {  // a wave stores one sub-tile
+        if constexpr (few_codes(SRC))
+            if (blocks > 8 * cus) return launch_few<CDT, MT, 2, SRC>(a, st);
         return launch_few<CDT, MT, 4, SRC>(a, st);
     } else {
         return launch_few<CDT, MT, 8, SRC>(a, st);
@@ -74,8 +76,18 @@ int launch_fp4_few(Fp4GemmArgs a, int bits, int c_dtype, hipStream_t st) {
 
 using namespace mx;
 
-// Which rows are quantized inside the product.
-static bool activation_rows_ok(int64_t M, int64_t K) { return M <= 16 ? K <= 8192 : M <= 32 && K <= 2048; }
+// Which activations are quantized inside the product: every workgroup does it again, which with more rows or more workgroups costs more than
+// the launch it saves; and only those whose codes would come here too, so that the sums over K are the same ones.  Kernels' us in two
+// launches / in one, weights from HBM, without the 1 to 10 us that lie between two launches:
+//             512 -> 4096   1536 -> 4096   1536 -> 8192   2048 -> 16384   8192 -> 8192   1536 -> 65536   4096 -> 131072
+//   M = 1       4.9 / 3.2      5.6 / 3.8      6.3 / 4.7      8.8 / 7.6     13.0 / 13.6     15.2 / 18.5     63.3 / 80.5
+//   8           5.3 / 3.6      5.8 / 4.3      6.6 / 5.2      9.7 / 8.6     16.2 / 15.4     19.0 / 19.0     67.0 / 84.9
+//   16          5.6 / 4.1      6.6 / 5.0      7.3 / 6.2     11.0 / 9.8     19.5 / 17.6     21.8 / 22.7     68.2 / 103
+//   32          6.1 / 5.4      7.3 / 6.9      8.4 / 11.8    14.0 / 18.0                    21.9 / 47.1
+static bool activations_pay(const Fp4GemmArgs &a) {
+    const int64_t cus = num_cus(), blocks = ((int64_t)a.N + 15) / 16;
+    return fp4_few_pays(a) && (a.M <= 16 ? a.K <= 8192 && blocks <= 4 * cus : a.M <= 32 && a.K <= 2048 && blocks <= cus);
+}
 
 extern "C" int mx_fp4_activation_gemm_nt(const void *x, int x_dtype, int64_t ldx, const uint8_t *bq, const uint8_t *b_scale, void *c, int c_dtype,
                                          int64_t M, int64_t N, int64_t K, int64_t ldb, int64_t ldbs, int64_t ldc, void *stream) {
@@ -85,11 +97,12 @@ extern "C" int mx_fp4_activation_gemm_nt(const void *x, int x_dtype, int64_t ldx
     if ((c_dtype != MX_BF16 && c_dtype != MX_FP16) || (x_dtype != c_dtype && x_dtype != MX_FP32)) return MX_EUNSUPPORTED;
     if (M == 0 || N == 0) return MX_OK;
     if (!c || (K && (!x || !bq || !b_scale))) return MX_EINVAL;
-    if (K == 0 || N > FP4_EXTENT || !activation_rows_ok(M, K) || !few_aligned(x, 16) || ldx * (x_dtype == MX_FP32 ? 4 : 2) % 16 || !few_aligned(bq, 16) || ldb % 16)
+    if (K == 0 || M > 32 || N > FP4_EXTENT || K > FP4_EXTENT || !few_aligned(x, 16) || ldx * (x_dtype == MX_FP32 ? 4 : 2) % 16 || !few_aligned(bq, 16) || ldb % 16)
         return MX_EUNSUPPORTED;
     hipStream_t st = (hipStream_t)stream;
     if (stream_is_capturing(st)) return MX_ECAPTURE;
-    Fp4GemmArgs a = {(const uint8_t *)x, nullptr, bq, b_scale, nullptr, nullptr, c, ldx, 0, 0, ldb, 0, ldbs, ldc, (int)M, (int)N, (int)K, 1, (int)M};
+    const Fp4GemmArgs a = {(const uint8_t *)x, nullptr, bq, b_scale, nullptr, nullptr, c, ldx, 0, 0, ldb, 0, ldbs, ldc, (int)M, (int)N, (int)K, 1, (int)M};
+    if (!activations_pay(a)) return MX_EUNSUPPORTED;
     if (x_dtype == MX_FP32) return c_dtype == MX_BF16 ? launch_few_rows<MX_BF16, MX_FP32>(a, st) : launch_few_rows<MX_FP16, MX_FP32>(a, st);
     return c_dtype == MX_BF16 ? launch_few_rows<MX_BF16, MX_BF16>(a, st) : launch_few_rows<MX_FP16, MX_FP16>(a, st);
 }
