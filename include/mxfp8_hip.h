@@ -734,8 +734,8 @@ int mx_fp4_gemm_nt(const uint8_t *aq, const uint8_t *a_scale, int a_format, cons
 
 /*
  * mx_quantize_rows of up to 32 rows of activations (in c_dtype, bf16 or fp16, or in fp32, rounded to it first) and mx_fp4_gemm_nt of them in
- * one launch, with the same bits.  MX_EUNSUPPORTED, with nothing launched, for more rows, longer ones, more columns than two calls
- * are slower for, or another layout: the caller takes the two calls.
+ * one launch, with the same bits.  MX_EUNSUPPORTED, with nothing launched, for more rows, longer ones, so many columns that two
+ * calls are quicker, or another layout: the caller takes the two calls.
  */
 int mx_fp4_activation_gemm_nt(const void *x, int x_dtype, int64_t ldx, const uint8_t *bq, const uint8_t *b_scale, void *c, int c_dtype,
                               int64_t M, int64_t N, int64_t K, int64_t ldb, int64_t ldbs, int64_t ldc, void *stream);

@@ -275,8 +275,8 @@ def add_rms_norm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor |
 
     ``x``: bf16 or fp16, its last axis a multiple of 8.  ``residual``: of ``x``'s shape, in ``x``'s type or in fp32; ``h`` has its type, and
     the norm reads the rounded ``h``.  ``out`` has ``x``'s type; for a 16-bit stream it is ``rms_norm(h, weight, eps)`` bit for bit.
-    ``weight``: the row's width in ``x``'s type or fp32, or ``None``.  Differentiable in all three,
-    in reverse mode.
+    ``weight``: the row's width in ``x``'s type or fp32, or ``None``.  Differentiable in all three
+    (reverse mode).
     """
     return _add_norm(x, residual, weight, eps, False)
 
